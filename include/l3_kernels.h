@@ -526,7 +526,8 @@ int l3_rot_embed_append(const void* qkv, const float* freq_table, void* q_out, v
  * A sequence may have no rows, and a row no token (rows before q_offsets[0] or from q_offsets[sequences] on; negative
  * positions, where a sequence has more rows than tokens): such rows come back as zeros and write nothing.  What the arrays
  * hold is not trusted with memory: lengths beyond the table's width count as that width, pages outside the cache as its
- * first or last.  Offsets that decrease give wrong values.
+ * first or last.  Where offsets decrease, attention returns zeros for every row, and the append takes a row for the first
+ * sequence's whose offsets enclose it.
  *   page_size   a power of two, at least 8; max_pages * page_size at most 2^30; rows at most 2^23, sequences at most
  *               L3_PAGED_MAX_SEQUENCES
  *   max_new     the most rows that any sequence has, where the caller knows it, else 0.  It chooses between kernels and

@@ -69,6 +69,7 @@ struct PagedGrid {
 struct Sequence {
     int row, n, kv;   // first row, rows, tokens
     int blocks;
+    bool falls;       // its offsets decrease
     __device__ __forceinline__ int past() const { return max(kv - n, 0); }
     // weight of the first j blocks
     __device__ __forceinline__ int64_t weight(int j, int positions) const {
@@ -140,6 +141,7 @@ struct Sequences {
         q.n = max(min(to, s.rows) - q.row, 0);
         q.kv = min(max(len, 0), s.max_kv);
         q.blocks = blocks_up_to(q.n);
+        q.falls = to < from;
         return q;
     }
     // Blocks whose rows are all among the first n: n / positions (the half keeps the product off the whole numbers).
@@ -168,9 +170,9 @@ struct Sequences {
         }
     }
     __device__ __forceinline__ Sequence at(int b) const {   // b is uniform
-        if (per_lane == 1) return {read_lane(own.row, b), read_lane(own.n, b), read_lane(own.kv, b), read_lane(own.blocks, b)};
+        if (per_lane == 1) return {read_lane(own.row, b), read_lane(own.n, b), read_lane(own.kv, b), read_lane(own.blocks, b), false};
         const Sequence q = sequence(b);
-        return {wave_uniform(q.row), wave_uniform(q.n), wave_uniform(q.kv), wave_uniform(q.blocks)};
+        return {wave_uniform(q.row), wave_uniform(q.n), wave_uniform(q.kv), wave_uniform(q.blocks), false};
     }
 };
 
@@ -203,7 +205,7 @@ struct Shares {
             }
             x -= read_lane(sum, kWaveSize - 1);
         }
-        return all.s.seqs - 1;   // (only with offsets that contradict themselves)
+        return all.s.seqs - 1;   // (the addends are those of the sum: one of the loop's steps has returned)
     }
 };
 
@@ -999,6 +1001,7 @@ struct WideItem {
     int t_first, t_stop;     // its tokens, or the piece's
     int slot;                // of the piece's partial result; -1: the block is whole
     int two;                 // two column blocks to a wavefront, or one
+    int falls;               // offsets decrease: no row is a sequence's
 };
 
 // Finds it out; for one wavefront (all four at it would take four times the issue slots, and a launch's workgroups begin
@@ -1008,20 +1011,28 @@ template <int HD, int WPE>
 __device__ __forceinline__ WideItem wide_item(const PagedAttnParams& p, const PagedGrid& grid) {
     using Time = WideTime<HD>;
     WideItem o;
-    o.rows = 0;
+    o.rows = o.falls = 0;
     Sequences sequences(p, 2 * kWaves);
 
     // The longest block, and all blocks' tiles to a compute unit, in blocks of two column blocks (of one: about twice as many).
     auto tiles_of = [](int tokens) { return (tokens + kTile - 1) / kTile; };
     int longest = 0;
     float weight = 0.f, blocks = 0.f;
+    bool falls = false;
     sequences.each([&](const Sequence& q) {
+        falls |= q.falls;
         if (q.blocks > 0) {
             longest = max(longest, tiles_of(q.kv));
             blocks += float(q.blocks);
             weight += float(q.blocks) * (float(q.past()) + 0.5f * float(sequences.positions) * float(q.blocks + 1));
         }
     });
+    // Only sequences that do not overlap have as many blocks as the launch has workgroups, and no piece without one.
+    if (__builtin_amdgcn_ballot_w64(falls) != 0) {
+        o.falls = 1;
+        if (grid.entries > 0 && blockIdx.x == 0) grid.cuts[0].pieces = 0;
+        return o;
+    }
     longest = wave_maximum(longest);
     const float per_unit = wave_sum(weight) * float(p.KVH) / float(grid.units * kTile);
     const float blocks_per_unit = wave_sum(blocks) * float(p.KVH) / float(grid.units);
@@ -1156,7 +1167,7 @@ attn_paged_wide_kernel(const PagedAttnParams p, const PagedGrid grid) {
         if (threadIdx.x == 0) s_item = item;
     }
     __syncthreads();
-    clear_other_rows<HD>(p, rows_begin, rows_end);
+    clear_other_rows<HD>(p, s_item.falls ? p.step.rows : rows_begin, rows_end);
     if (s_item.rows == 0) return;
     WideItem o = s_item;
     o.b = wave_uniform(o.b); o.kvh = wave_uniform(o.kvh); o.kv = wave_uniform(o.kv);
@@ -1189,9 +1200,15 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
     // places where consecutive parts cut a block are different tiles; where nothing is cut what a block of 16 tokens does, so
     // that none but the shortest share a part as long as there are enough (one sequence of 30 tokens 8.0 us otherwise, 5.9).  Whole eights, where there are as many, and consecutive
     // parts on one XCD: what a kv head's blocks share then stays in its cache.
-    auto weight_of = [&](const Sequence& q) { return q.weight(q.blocks, positions); };
+    // Only sequences that do not overlap keep the weights within 64 bits: where offsets decrease the line is empty.
+    bool falls = false;
+    auto weight_of = [&](const Sequence& q) {
+        falls |= q.falls;
+        return q.weight(q.blocks, positions);
+    };
     const Shares<int64_t, decltype(weight_of)> line(sequences, weight_of);
-    const int64_t total = line.total * p.KVH;
+    const bool overlap = __builtin_amdgcn_ballot_w64(falls) != 0;
+    const int64_t total = overlap ? 0 : line.total * p.KVH;
     int parts = int(std::max<int64_t>(1, std::min<int64_t>(gridDim.x, total / (grid.slots ? kLeastChunk : kBlockWeight + 16))));
     if (parts >= kXcds) parts &= ~(kXcds - 1);
     const int mine = id < parts && parts >= kXcds ? (id % kXcds) * (parts / kXcds) + id / kXcds : id;
@@ -1200,7 +1217,7 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
         if (id == 0) grid.cuts[0].pieces = parts;
     }
 
-    clear_other_rows<HD>(p, rows_begin, rows_end);
+    clear_other_rows<HD>(p, overlap ? s.rows : rows_begin, rows_end);
     if (total == 0 || id >= parts) return;
 
     const int64_t per_part = quotient(total, parts);
@@ -1258,7 +1275,7 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
             j = 0;
             if (++b == s.seqs) {
                 b = 0;
-                if (++kvh >= p.KVH) return;   // (only with offsets that contradict themselves)
+                if (++kvh >= p.KVH) return;   // (the line's end is the last head's: begin has reached `end`)
             }
             seq = sequences.at(b);
         }

@@ -2,7 +2,8 @@
 // and pages of a power of two tokens.  All of it lies on the device, so that a recorded launch serves any step.
 //
 // Nothing here trusts what the arrays hold with memory: offsets are clamped to the rows, lengths to the page table's width,
-// pages to the cache.  (Arrays that contradict themselves give wrong values, not accesses out of range.)
+// pages to the cache.  Offsets that decrease would have more blocks than attention's launch has workgroups: it finds them and
+// takes every row for nobody's.  (The append takes a row for the first sequence's whose offsets enclose it.)
 #pragma once
 
 #include "l3_device.hpp"
