@@ -1317,7 +1317,10 @@ __device__ __forceinline__ void merge_pieces(const PagedAttnParams& p, const Cut
             }
         }
     }
-    const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;   // (a row that sees nothing)
+    // A block that was cut has more tokens than rows and its last row sees them all, so every row sees some: the sum is 0 only
+    // where all their scores are minus infinity, and the row NaN then, as in a block that was not cut.
+    static_assert(kLeastWidePiece * kTile > 8 * 16 && 2 * kLeastPiece > 2 * 16, "tokens of a block that is cut; rows of a block");
+    const float inv = 1.0f / total;
     uint16_t* const out = p.out + int64_t(row) * p.o_sr + h * p.o_sh + dim;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
