@@ -76,6 +76,7 @@ class PagedServer:
             for _ in range(2))
         self.free = deque(range(pages))
         self.graphs = {} if graphs and dev.type == "cuda" else None      # rows -> what _record returns
+        self._recorded_of = None
         self.steps = {"mixed": 0, "generating": 0}
 
     # ------------------------------------------------------------------ one step on the device
@@ -111,6 +112,17 @@ class PagedServer:
         h = h[0] if every_row else h[0].index_select(0, step.last_rows)
         logits = m._linear(h, m.wte)
         return ops.argmax(logits) if hasattr(ops, "argmax") else torch.argmax(logits, dim=-1)
+
+    def _drop_outdated(self):
+        """Recorded steps hold the model's tensors by address and the choice of its linears: they go when either is another.
+        (Looked at once per generate(): the model stays as it is during one.)"""
+        m = self.model
+        tensors = [m.wte, m.ln_f, m.freqs_cis, *(t for L in m.layers for name, t in L.items() if not name.startswith("cache_"))]
+        now = m.ops, m.decode_linear_rows, [(t.data_ptr(), t.shape, t.stride()) for t in tensors]
+        if now != self._recorded_of:
+            if self.graphs:
+                self.graphs.clear()
+            self._recorded_of = now
 
     def _run(self, plan):
         rows = sum(n for _, n in plan)
@@ -178,6 +190,7 @@ class PagedServer:
     def generate(self, prompt_tokens, max_gen_len, echo=False, ignore_eos=False):
         """Greedy answers of LlamaDecoder.generate (each prompt a non-empty list of ids), requests admitted in order as pages
         become free."""
+        self._drop_outdated()
         c, stop = self.model.config, set(self.model.tokenizer.stop_tokens)
         requests = [_Request(i, p, min(c.block_size, len(p) + max_gen_len)) for i, p in enumerate(prompt_tokens)]
         for r in requests:

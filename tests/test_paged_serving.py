@@ -140,3 +140,52 @@ def test_model_with_head_norms_matches_cpu_logits(gpu):
         with pytest.raises(NotImplementedError):
             dut.generate_graphed(ids.tolist(), 4)
         assert [len(t) for t in dut.generate(ids.tolist(), 4, ignore_eos=True)] == [4] * rows
+
+
+def test_recorded_steps_go_with_the_model_they_were_recorded_of():
+    m = model(tiny_config(qk_norm=True), CpuOps, "cpu", torch.float32)
+    server = PagedServer(m, 4, page_size=8)
+    server.graphs = {}
+    server.generate([], 1)
+
+    def changes():
+        m.decode_linear_rows = 8
+        yield
+        m.layers[1]["c_proj"] = m.layers[1]["c_proj"].clone()
+        yield
+        m.layers[0]["k_norm"] = m.layers[0]["k_norm"].clone()
+        yield
+        m.ln_f = m.ln_f.clone()
+        yield
+        m.wte = torch.zeros(m.wte.shape[0], m.wte.shape[1] + 8)[:, :-8].copy_(m.wte)
+        yield
+        m.ops = type("Others", (CpuOps,), {})
+        yield
+
+    for _ in changes():
+        server.graphs[4] = (None, None, None)
+        server.generate([], 1)
+        assert not server.graphs
+        server.graphs[4] = (None, None, None)
+        server.generate([], 1)      # nothing is another: recorded steps stay
+        assert server.graphs
+
+
+@pytest.mark.gpu
+def test_a_server_answers_with_the_models_present_weights(gpu):
+    """The steps it had recorded read the weights that were replaced (kept alive here)."""
+    from custom_kernels import custom_kernels_extension as cke
+
+    cfg = tiny_config(n_head=4, n_kv_head=2, n_embd=256)
+    dut, other = (model(cfg, cke, gpu, torch.bfloat16, seed=s) for s in (7, 8))
+    server = PagedServer(dut, 64, page_size=8)
+    first = server.generate(PROMPTS, 8, ignore_eos=True)
+    kept = dut.wte, dut.layers
+    dut.wte, dut.layers = other.wte, other.layers
+    want = PagedServer(other, 64, page_size=8).generate(PROMPTS, 8, ignore_eos=True)
+    print("weights replaced under a server with recorded steps", flush=True)
+    assert server.generate(PROMPTS, 8, ignore_eos=True) == want != first
+    dut.wte, dut.layers = kept
+    dut.set_decode_linear_rows(0)
+    want = PagedServer(dut, 64, page_size=8).generate(PROMPTS, 8, ignore_eos=True)
+    assert server.generate(PROMPTS, 8, ignore_eos=True) == want
