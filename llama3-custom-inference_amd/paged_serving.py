@@ -91,7 +91,7 @@ class PagedServer:
             return ops.flash_attention_paged(q, self.k_pages[i], self.v_pages[i], *where, max_new)
 
         x = F.embedding(step.tokens, m.wte)
-        if every_row and m.decode_linear_rows > 0 and m.FUSED_MAX_ROWS < step.rows <= m.QKV_FUSED_MAX_ROWS and hasattr(ops, "linear_splitk"):
+        if every_row and m.decode_linear_rows > 0 and m.FUSED_MAX_ROWS < step.rows <= m.QKV_FUSED_MAX_ROWS and self._streaming_linears():
             # the linears of a dense decode step of as many sequences
             x = x.unsqueeze(1)
             h = ops.rms_norm(x, m.layers[0]["ln_1"], c.norm_eps)
@@ -112,6 +112,13 @@ class PagedServer:
         h = h[0] if every_row else h[0].index_select(0, step.last_rows)
         logits = m._linear(h, m.wte)
         return ops.argmax(logits) if hasattr(ops, "argmax") else torch.argmax(logits, dim=-1)
+
+    def _streaming_linears(self):
+        """Whether the linears of 5 to 64 rows take the model's projections: whole chunks of 128 and dense 16-byte rows.  (The
+        other steps' linears take more; LlamaDecoder._swiglu and _vocabulary see to theirs.)"""
+        return hasattr(self.model.ops, "linear_splitk") and all(
+            w.shape[1] % 128 == 0 and w.shape[0] % 8 == 0 and w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0
+            for L in self.model.layers for w in (L["c_attn"], L["c_proj"], L["mlp_proj"]))
 
     def _drop_outdated(self):
         """Recorded steps hold the model's tensors by address and the choice of its linears: they go when either is another.

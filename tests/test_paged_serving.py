@@ -189,3 +189,38 @@ def test_a_server_answers_with_the_models_present_weights(gpu):
     dut.set_decode_linear_rows(0)
     want = PagedServer(dut, 64, page_size=8).generate(PROMPTS, 8, ignore_eos=True)
     assert server.generate(PROMPTS, 8, ignore_eos=True) == want
+
+
+def chosen_tokens_are_near_the_best(ref, prompts, answers, length):
+    """The bound of test_hip_operators_in_the_loop_choose_the_cpu_models_tokens, with one pass over each text."""
+    for prompt, answer in zip(prompts, answers):
+        assert len(answer) == length
+        for i, token in enumerate(answer):
+            with torch.inference_mode():
+                logits = ref.forward(torch.tensor([prompt + answer[:i]]))[0, -1]
+            assert logits[token] >= logits.max() - 2 * 0.04 * logits.abs().max(), (len(prompt), i)
+
+
+def transposed(w):
+    return w.t().contiguous().t()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what,sequences", [("width", 7), ("width", 20), ("transposed", 20)])
+def test_generating_steps_of_weights_that_the_streaming_linears_refuse(gpu, what, sequences):
+    """Widths that are no multiple of 128, and weights that lie the other way round (which steps of more than 16 rows take
+    everywhere else): such a model's generating steps take the linears that its other steps take."""
+    from custom_kernels import custom_kernels_extension as cke
+
+    cfg = tiny_config(n_head=3, n_kv_head=1, n_embd=192, hidden_dim=320) if what == "width" else tiny_config()
+    dut = model(cfg, cke, gpu, torch.bfloat16, seed=7)
+    ref = la.LlamaDecoder(cfg, CpuOps, "cpu", dtype=torch.float32, weights_from=dut)
+    for L in dut.layers if what == "transposed" else ():
+        for name in ("c_attn", "c_proj", "mlp_proj"):
+            L[name] = transposed(L[name])
+    prompts = [la.random_prompts(1, 18 if what == "transposed" else 3 + i % 4, 900, i)[0] for i in range(sequences)]
+    for graphs in (False, True):
+        print(f"{what}, {sequences} sequences, graphs {graphs}", flush=True)
+        server = PagedServer(dut, 80, page_size=8, max_sequences=sequences, graphs=graphs)
+        chosen_tokens_are_near_the_best(ref, prompts, server.generate(prompts, 4, ignore_eos=True), 4)
+        assert server.graphs is None or [entry[0] is not None for entry in server.graphs.values()] == [True]
