@@ -15,6 +15,7 @@ takes every prompt's tokens behind the shortest one's length one by one, gives 6
 """
 
 import gc
+import threading
 from collections import deque
 
 import torch
@@ -60,7 +61,8 @@ class _Step:
 
 class PagedServer:
     """model: a LlamaDecoder whose operator module has the paged operators.  pages x page_size tokens of cache per layer;
-    at most `max_sequences` requests at once and `max_rows` new tokens in a step."""
+    at most `max_sequences` requests at once and `max_rows` new tokens in a step.  The pages, the steps' tensors and the recorded
+    steps are those of one generate() at a time: calls from several threads take turns."""
 
     def __init__(self, model: LlamaDecoder, pages: int, page_size: int = 64, max_sequences: int = 64, max_rows: int = 2048,
                  graphs: bool = True):
@@ -77,6 +79,7 @@ class PagedServer:
         self.free = deque(range(pages))
         self.graphs = {} if graphs and dev.type == "cuda" else None      # rows -> what _record returns
         self._recorded_of = None
+        self._turn = threading.Lock()
         self.steps = {"mixed": 0, "generating": 0}
 
     # ------------------------------------------------------------------ one step on the device
@@ -193,10 +196,13 @@ class PagedServer:
                 plan.append((r, n))
         return plan
 
-    @torch.inference_mode()
     def generate(self, prompt_tokens, max_gen_len, echo=False, ignore_eos=False):
         """Greedy answers of LlamaDecoder.generate (each prompt a non-empty list of ids), requests admitted in order as pages
         become free."""
+        with self._turn, torch.inference_mode():
+            return self._generate(prompt_tokens, max_gen_len, echo, ignore_eos)
+
+    def _generate(self, prompt_tokens, max_gen_len, echo, ignore_eos):
         self._drop_outdated()
         c, stop = self.model.config, set(self.model.tokenizer.stop_tokens)
         requests = [_Request(i, p, min(c.block_size, len(p) + max_gen_len)) for i, p in enumerate(prompt_tokens)]

@@ -2,6 +2,8 @@
 the oracle, token for token against LlamaDecoder.generate.  GPU: the HIP operators in the loop, eager and recorded, every chosen
 token against the logits that the float32 CPU model gives the same text."""
 
+import threading
+
 import pytest
 import torch
 
@@ -224,3 +226,32 @@ def test_generating_steps_of_weights_that_the_streaming_linears_refuse(gpu, what
         server = PagedServer(dut, 80, page_size=8, max_sequences=sequences, graphs=graphs)
         chosen_tokens_are_near_the_best(ref, prompts, server.generate(prompts, 4, ignore_eos=True), 4)
         assert server.graphs is None or [entry[0] is not None for entry in server.graphs.values()] == [True]
+
+
+def test_calls_from_several_threads_take_turns():
+    """The second call comes while the first holds every page and has a step half done."""
+    m = model(tiny_config(), CpuOps, "cpu", torch.float32)
+    want = [m.generate([p], 6, ignore_eos=True)[0] for p in PROMPTS[:2]]
+    server, answers, errors, began = PagedServer(m, 2, page_size=8), {}, [], threading.Event()
+
+    def call(i):
+        try:
+            answers[i] = server.generate([PROMPTS[i]], 6, ignore_eos=True)[0]
+        except Exception as e:      # noqa: BLE001 (shown below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(2)]
+
+    def interrupted(*a):
+        if not began.is_set():
+            began.set()
+            threads[1].start()
+            threads[1].join(0.5)      # it is through only if it did not wait for this call
+        return CpuOps.flash_attention_paged(*a)
+
+    m.ops = type("Interrupted", (CpuOps,), {"flash_attention_paged": staticmethod(interrupted)})
+    threads[0].start()
+    for t in threads:
+        began.wait(10)
+        t.join(10)
+    assert not errors and answers == dict(enumerate(want)) and sorted(server.free) == [0, 1]
