@@ -90,3 +90,14 @@ def test_more_rows_than_a_launch_holds():
     heads = 512
     assert attend(step(rows=rows, sequences=60000), heads=(heads, heads, 64), qs=(heads * 64, 64), os=(heads * 64, 64),
                   ks=(16 * heads * 64, heads * 64, 64), vs=(16 * heads * 64, heads * 64, 64)) == SHAPE
+
+
+@pytest.mark.parametrize("rows,max_pages,max_new", [(5, 64, 1), (5, 64, 0), (300, 256, 0), (300, 256, 300)])
+def test_a_workspace_of_a_step_that_may_be_cut_is_checked(rows, max_pages, max_new):
+    """Page tables wide enough for both forms to cut blocks."""
+    s = step(rows=rows, max_pages=max_pages, table_stride=max_pages, max_new=max_new)
+    needed = _l3lib.load().l3_attn_paged_workspace_bytes(s, 8, 2, 64)
+    assert needed > 0
+    for nbytes in (0, 1, needed - 1):
+        assert attend(s, ws=FAKE, nbytes=nbytes) == WORKSPACE
+    assert attend(s, ws=FAKE + 128, nbytes=needed) == ALIGNMENT
