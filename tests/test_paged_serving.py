@@ -255,3 +255,20 @@ def test_calls_from_several_threads_take_turns():
         began.wait(10)
         t.join(10)
     assert not errors and answers == dict(enumerate(want)) and sorted(server.free) == [0, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("requests,sequences,qk_norm", [(20, 20, False), (23, 20, True), (64, 64, False), (64, 64, True), (70, 64, False)])
+def test_generating_steps_of_many_sequences(gpu, requests, sequences, qk_norm, graphs):
+    """Steps of 17 to 64 rows have linears of their own; 20 sequences make a step that is no power of two."""
+    from custom_kernels import custom_kernels_extension as cke
+
+    cfg = tiny_config(n_head=4, n_kv_head=2, n_embd=256, qk_norm=qk_norm)
+    dut = model(cfg, cke, gpu, torch.bfloat16, seed=7)
+    ref = la.LlamaDecoder(cfg, CpuOps, "cpu", dtype=torch.float32, weights_from=dut)
+    prompts = [la.random_prompts(1, 1 + 5 * i % 23, 900, i)[0] for i in range(requests)]
+    print(f"{requests} requests, {sequences} at once, norms {qk_norm}, graphs {graphs}", flush=True)
+    server = PagedServer(dut, 64 * 4, page_size=8, max_sequences=sequences, max_rows=512, graphs=graphs)
+    chosen_tokens_are_near_the_best(ref, prompts, server.generate(prompts, 4, ignore_eos=True), 4)
+    assert not graphs or sequences in server.graphs and all(entry[0] is not None for entry in server.graphs.values())
