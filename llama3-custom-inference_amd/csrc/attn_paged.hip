@@ -997,11 +997,10 @@ struct WideTime {
 // What a workgroup of a wide launch does.
 struct WideItem {
     int b, kvh, kv;          // sequence, kv head, tokens of the sequence
-    int row, rows, first;    // the block: first row, rows (0: there is nothing to do), position of the first row
+    int row, rows, first;    // the block: first row, rows (0: nothing to do, -1: no row is a sequence's), position of the first row
     int t_first, t_stop;     // its tokens, or the piece's
     int slot;                // of the piece's partial result; -1: the block is whole
     int two;                 // two column blocks to a wavefront, or one
-    int falls;               // offsets decrease: no row is a sequence's
 };
 
 // Finds it out; for one wavefront (all four at it would take four times the issue slots, and a launch's workgroups begin
@@ -1011,7 +1010,7 @@ template <int HD, int WPE>
 __device__ __forceinline__ WideItem wide_item(const PagedAttnParams& p, const PagedGrid& grid) {
     using Time = WideTime<HD>;
     WideItem o;
-    o.rows = o.falls = 0;
+    o.rows = 0;
     Sequences sequences(p, 2 * kWaves);
 
     // The longest block, and all blocks' tiles to a compute unit, in blocks of two column blocks (of one: about twice as many).
@@ -1029,7 +1028,7 @@ __device__ __forceinline__ WideItem wide_item(const PagedAttnParams& p, const Pa
     });
     // Only sequences that do not overlap have as many blocks as the launch has workgroups, and no piece without one.
     if (__builtin_amdgcn_ballot_w64(falls) != 0) {
-        o.falls = 1;
+        o.rows = -1;
         if (grid.entries > 0 && blockIdx.x == 0) grid.cuts[0].pieces = 0;
         return o;
     }
@@ -1167,7 +1166,11 @@ attn_paged_wide_kernel(const PagedAttnParams p, const PagedGrid grid) {
         if (threadIdx.x == 0) s_item = item;
     }
     __syncthreads();
-    clear_other_rows<HD>(p, s_item.falls ? p.step.rows : rows_begin, rows_end);
+    if (s_item.rows < 0) {
+        clear_other_rows<HD>(p, p.step.rows, p.step.rows);
+        return;
+    }
+    clear_other_rows<HD>(p, rows_begin, rows_end);
     if (s_item.rows == 0) return;
     WideItem o = s_item;
     o.b = wave_uniform(o.b); o.kvh = wave_uniform(o.kvh); o.kv = wave_uniform(o.kv);
@@ -1207,8 +1210,12 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
         return q.weight(q.blocks, positions);
     };
     const Shares<int64_t, decltype(weight_of)> line(sequences, weight_of);
-    const bool overlap = __builtin_amdgcn_ballot_w64(falls) != 0;
-    const int64_t total = overlap ? 0 : line.total * p.KVH;
+    if (__builtin_amdgcn_ballot_w64(falls) != 0) {
+        if (grid.slots && tid == 0 && id == 0) grid.cuts[0].pieces = 0;
+        clear_other_rows<HD>(p, s.rows, s.rows);
+        return;
+    }
+    const int64_t total = line.total * p.KVH;
     int parts = int(std::max<int64_t>(1, std::min<int64_t>(gridDim.x, total / (grid.slots ? kLeastChunk : kBlockWeight + 16))));
     if (parts >= kXcds) parts &= ~(kXcds - 1);
     const int mine = id < parts && parts >= kXcds ? (id % kXcds) * (parts / kXcds) + id / kXcds : id;
@@ -1217,7 +1224,7 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
         if (id == 0) grid.cuts[0].pieces = parts;
     }
 
-    clear_other_rows<HD>(p, overlap ? s.rows : rows_begin, rows_end);
+    clear_other_rows<HD>(p, rows_begin, rows_end);
     if (total == 0 || id >= parts) return;
 
     const int64_t per_part = quotient(total, parts);
