@@ -7,7 +7,10 @@
 //   S[tokens x 16 columns] = K Q^T,   O^T[dims x 16 columns] += V^T P     (v_mfma_f32_16x16x32_bf16)
 //
 // Softmax with a running maximum: scores, maxima, sums and outputs are float32; the weights exp(s - m) alone are rounded, to the
-// bf16 that the matrix instructions take (2^-9 of a weight, errors of all tokens independent: below the rounding of the output).
+// bf16 that the matrix instructions take (2^-9 of a weight, errors of all tokens independent: below the rounding of the output;
+// over N(0, 1) values 0.0020 to 0.0023 of the result's norm in all, 0.0016 to 0.0017 with float32 weights).  The denominator is a float32 sum,
+// in the narrow form of the weights before that rounding, as in the dense decode kernels, in the wide form of the rounded ones,
+// which the matrix pipe adds up on its way.
 //
 // A block is what one workgroup of four wavefronts takes.  Narrow: 16 or 32 columns, whose tokens the wavefronts share out
 // among themselves, each with a softmax of its own (a sequence with a single or a few new tokens, bound by the bytes of its
@@ -989,8 +992,11 @@ struct WideTime {
     static constexpr float alone2 = HD == 64 ? 1.12f : 1.40f, full2 = HD == 64 ? 0.46f : 0.90f;
     static constexpr float start = 0.7f;   // of a workgroup, its share of a unit
     static constexpr float merge = 8.0f;   // the last launch, and partial results written
-    // Pieces to a unit where blocks are cut.  A fourth of four residents adds little and its partial result costs what the others'
-    // do (head size 64, pieces of three prompts beside generating sequences: 66 us with four, 58 with three).
+    // Pieces to a unit where blocks are cut: a choice between calls, none is best for all.  us with 2, 3 (taken), 4 at head size 64:
+    // three prompts' pieces beside 13 generating sequences 67, 60, 67; two beside 30 of them 75, 68, 68; one beside 8 of 8000
+    // tokens 44, 48, 44; 512 of 4096 tokens, 300 of 2500, 4 x 200 of 3000, 24 x 12 of 500 to 4000: within 1.  With 1, 2 (taken), 3 at
+    // 128: three beside 13 98, 107, 97; 512 of 7012 tokens 99, 73, 92; 2 x 700 of 5000 144, 148, 149; 4 x 200 of 3000 66, 79, 74; 24 x 12 of
+    // 500 to 4000 53, 56, 55.
     static constexpr int pieces = HD == 64 ? 3 : 2;
 };
 
@@ -1117,7 +1123,9 @@ __device__ __forceinline__ WideItem wide_item(const PagedAttnParams& p, const Pa
         if (o.b > 0) x -= read_lane(upto, o.b - 1);
         seq = sequences.at(o.b);
         j = read_lane(from, o.b) + x;
-    } else {   // too many sequences for that: the longest of each first
+    } else {   // more sequences than lanes: not in order of their length, but the longest of each first (64 sequences, us in order
+               // and, with an empty one more, out of it: prompts of 30 to 700 tokens 61, 66; of 30 to 2000 194, 199, at head size
+               // 128 387, 396; three prompts' pieces beside 61 single rows 78, 88, at 128 116, 160)
         int x = item - cut.total;
         o.b = wave_uniform(whole.find(x));
         seq = sequences.at(o.b);
@@ -1146,8 +1154,8 @@ __device__ __forceinline__ WideItem wide_item(const PagedAttnParams& p, const Pa
     return o;
 }
 
-// Wide blocks.  Bound by the matrix pipe at head size 128 (2048 rows behind 14336 tokens, 32/8 heads: 468 us, 1.10 PFLOP/s; a large
-// matrix product reaches 1.23) and by the vector instructions of the softmax beside it at 64, where a tile's 32 exponentials
+// Wide blocks.  Bound by the matrix pipe at head size 128 (2048 rows behind 14336 tokens, 32/8 heads: 460 us, 1.12 PFLOP/s, 478 on
+// another device; a large matrix product reaches 1.23) and by the vector instructions of the softmax beside it at 64, where a tile's 32 exponentials
 // a lane, at a quarter of the vector rate, take nearly as long as its 36 matrix instructions (4096 rows behind 4096 tokens: 249
 // us, 0.83 PFLOP/s).  Short calls are their start: workgroups begin over 4 us, find their item, and have their first tile 2.4 us later
 // (eight prompts of 134 to 1120 tokens: 29 us, of which the tiles are 11).  Four or two workgroups share a compute unit, so
@@ -1186,7 +1194,7 @@ attn_paged_wide_kernel(const PagedAttnParams p, const PagedGrid grid) {
 // 128, 477 MB in 80 us (6.0 TB/s; a pure read reaches 6.7), three of 60000 to 131071 tokens 1.07 GB in 166 us (6.4).  Every
 // tile's loads are in flight while the one before is multiplied; two workgroups to a compute unit keep some 64 KiB on their way.
 // One part a workgroup, all of one weight: none ends long before the others.  What is not tiles is 3 us of search in front and
-// the last launch, 4 to 6 us (24 sequences with 2 to 7 drafted rows: 160 MB, 33 + 6 us).
+// the last launch, 4 to 6 us (24 sequences with 2 to 7 drafted rows: 160 MB, 38 + 6 us).
 template <int HD, int LOADS, int CB, int WPE>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
@@ -1201,7 +1209,7 @@ attn_paged_narrow_kernel(const PagedAttnParams p, const PagedGrid grid) {
 
     // How many parts: one per workgroup, fewer where there is little to do.  A part weighs at least kLeastChunk, so that the
     // places where consecutive parts cut a block are different tiles; where nothing is cut what a block of 16 tokens does, so
-    // that none but the shortest share a part as long as there are enough (one sequence of 30 tokens 8.0 us otherwise, 5.9).  Whole eights, where there are as many, and consecutive
+    // that none but the shortest share a part as long as there are enough (one sequence of 30 tokens 8.0 us otherwise, 5.4).  Whole eights, where there are as many, and consecutive
     // parts on one XCD: what a kv head's blocks share then stays in its cache.
     // Only sequences that do not overlap keep the weights within 64 bits: where offsets decrease the line is empty.
     bool falls = false;
@@ -1390,14 +1398,22 @@ Sizes sizes_of(const PagedStep& s, int QH, int KVH, int HD, int max_new) {
     const int R = QH / KVH, ppb = 16 / R, cus = current_device_cus();
     const int64_t rows = max_new > 0 ? std::min(max_new, s.rows) : s.rows;   // of a sequence at most
     Sizes z = {};
+    // Narrow up to two column blocks (more would be two streams of the same tokens).  us of the narrow and of the wide form, rows to
+    // a sequence on either side of the line: head size 128, four heads to a kv head, 24 sequences of 500 to 4001 tokens: 4 rows 46, 51;
+    // 8 rows 50, 53; 9 rows 75, 56; 16 rows 81, 59; 4 sequences of 1500: 8 rows 21, 30; 9 rows 22, 31; 16 rows 24, 31.  Head size 64: 8 rows 31,
+    // 26; 9 rows 41, 28; of 4 sequences 15, 22; 15, 21.  Sixteen heads to a kv head, 128: 2 rows 33, 27; 3 rows 44, 31; of 4 sequences 19,
+    // 30; 19, 31.  One head, 128: 32 rows 50, 52; 33 rows 76, 55; of 4 sequences 21, 30; 23, 31.  (Few sequences would have the narrow form a
+    // little further: how many there are is known, how long they are is not.)
     if (rows <= 2 * ppb) {
         z.narrow = rows > ppb ? 2 : 1;
         z.workgroups = z.entries = kNarrowWpe * cus / kXcds * kXcds;
-        if (s.max_kv <= kLeastCut) z.entries = 0;   // few tokens: what a cut saves is less than the last launch costs
+        // few tokens: what a cut saves is less than the last launch costs (by the table: one of 30 tokens has it at 8192, 9.6 us for 5.2)
+        if (s.max_kv <= kLeastCut) z.entries = 0;
         z.slots = size_t(z.entries) * 2 * narrow_slot_bytes(HD, z.narrow);
     } else {
         // blocks: every sequence may end with one that is not full.  Pieces: at most four to a compute unit; where the
-        // blocks alone keep the device busy none is cut.
+        // blocks alone keep the device busy none is cut, however long one of them (head size 128, 8 kv heads, a piece of 300 rows
+        // beside one row behind 131071 tokens and 200 of 500: 213 us; 260 of them are that many blocks: 2.3 ms).
         auto blocks_of = [&](int cb) { return (s.rows / (ppb * kWaves * cb) + std::min(s.seqs, s.rows)) * int64_t(KVH); };
         const int residents = wide_wpe(HD) * cus;
         if (blocks_of(2) < 4 * residents && s.max_kv > kLeastWideCut) z.entries = 4 * cus;

@@ -55,7 +55,7 @@ struct AppendParams {
 // A workgroup has one row; a thread the same chunk of every (256 / VPR)th head.  Bound by bytes: four prompts of 1500 to 2600
 // tokens, 32/8 heads of 128, 192 MB in 34 us (5.6 TB/s; the counters show 98 MB read and 94 written); pieces of 1 to 601
 // tokens, 28 MB, 9 us, of which 3 are the launch and the way to the first load: place, page and row are three trips to memory, which
-// other rows' workgroups cover (rows requested ahead of their place: no faster).  A single row: 2.4 us.
+// other rows' workgroups cover (rows requested ahead of their place: no faster).  A single row: 2.2 us.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) rot_embed_append_paged_kernel(const AppendParams p) {
     constexpr int VPR = HD / 8, HEADS = kThreads / VPR;

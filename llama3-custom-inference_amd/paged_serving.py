@@ -9,13 +9,17 @@ What a step works with lies in device tensors (tokens, q_offsets, kv_lens, page_
 one copy from the host.  A step in which every request generates has one row for each and is replayed from a HIP graph, recorded
 once per number of rows rounded up to a power of two; rows beyond the requests are no sequence's token.
 
-Measured on the 1B architecture, 64 requests of 16 .. 1000 prompt ids (five lengths, drawn) and 128 greedy tokens each: 26.1 k
-generated tokens/s with 512 rows to a step, 33.8 k with 2048, 36.2 k with 8192 (prompt passes included).  generate_graphed, which
-takes every prompt's tokens behind the shortest one's length one by one, gives 6.2 k on the same requests.
+Measured on the 1B architecture (python paged_serving.py), 64 requests of 16 .. 1000 prompt ids (five lengths, drawn) and 128
+greedy tokens each: 26.4 k generated tokens/s with 512 rows to a step, 33.8 k with 2048, 36.4 k with 8192 (prompt passes included).
+generate_graphed, which takes every prompt's tokens behind the shortest one's length one by one, gives 6.2 k on the same requests.
+One request alone: 1.15 k, generate_graphed 1.9 k (up to four sequences its step is one launch; the steps here are operators one by
+one).
 """
 
 import gc
+import random
 import threading
+import time
 from collections import deque
 
 import torch
@@ -243,3 +247,29 @@ class PagedServer:
     def _release(self, request):
         self.free.extend(request.pages)
         request.pages = []
+
+
+def timed_serving(generate, prompts, max_gen_len, repeats=3):
+    """Generated tokens/s of a generate(prompts, max_gen_len, ignore_eos=True), prompt passes included: best of `repeats` behind
+    one that records the steps."""
+    best = 0.0
+    for i in range(repeats + 1):
+        torch.cuda.synchronize()
+        begin = time.perf_counter()
+        answers = generate(prompts, max_gen_len, ignore_eos=True)      # (ends with the last tokens on the host)
+        if i > 0:
+            best = max(best, sum(map(len, answers)) / (time.perf_counter() - begin))
+    return best
+
+
+if __name__ == "__main__":      # the figures above
+    from custom_kernels import custom_kernels_extension
+    from llama_arch import LlamaConfig, random_prompts
+
+    draw = random.Random(0)
+    every_prompt = [random_prompts(1, draw.choice((16, 64, 200, 500, 1000)), 128000, i)[0] for i in range(64)]
+    model = LlamaDecoder(LlamaConfig(max_model_len=1300, max_gen_batch_size=64), custom_kernels_extension, "cuda")
+    for prompts in every_prompt, every_prompt[:1]:
+        loops = {f"{rows} rows to a step": PagedServer(model, len(prompts) * 20, max_rows=rows).generate for rows in (512, 2048, 8192)}
+        for name, generate in {**loops, "generate_graphed": model.generate_graphed}.items():
+            print(f"{len(prompts)} requests, {name}: {timed_serving(generate, prompts, 128):.0f} tokens/s", flush=True)
