@@ -546,7 +546,8 @@ typedef struct l3_paged_step {
  * Causal grouped-query attention of a step's rows over their sequences' pages:
  *   out[r, h, :] = sum_{j <= p(r)} softmax_j(scale * q[r, h, :] . k_j) v_j,   p(r) the row's position
  * where k_j, v_j are token j of the row's sequence and kv head h / (QH / KVH).  The step's own keys and values are in the
- * cache already (l3_rot_embed_append_paged).
+ * cache already (l3_rot_embed_append_paged).  Products q . k_j below -1e30 count as minus infinity; a row that has no other is
+ * NaN.
  *   q, out            (rows, QH, HD) bf16 with {row, head} strides
  *   k_pages, v_pages  (pages, page_size, KVH, HD) bf16 with {page, token, head} strides; HD contiguous, all strides
  *                     multiples of 8, token strides below 2^24 elements, pointers 16-byte aligned
